@@ -51,6 +51,12 @@ PyObject* guarded(const F& f) {
   }
 }
 
+// What a kernel wrote to through its address counts as changed in place: the version by which autograd and
+// whoever remembers something of a tensor know it (inference tensors have none).
+void mark_written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Span {
   uintptr_t begin, end;
   uint32_t i;
@@ -85,6 +91,7 @@ bool spans_meet(std::vector<Span>& spans, const std::vector<size_t>& list_ends, 
 // What is asked of lists of tensors.  The first n_written are written, the others read.
 struct Lists {
   size_t n = 0;
+  std::vector<std::vector<const at::Tensor*>> ts;
   std::vector<std::vector<int64_t>> ptrs;  // per list, as the C entry points take them
   std::vector<std::vector<int32_t>> dtypes;
   std::vector<int64_t> counts;             // of the first list
@@ -95,7 +102,7 @@ struct Lists {
 
   // False with a Python error set where a list holds something else.
   bool look(PyObject* const* lists, size_t n_lists, int device, int n_written, bool in_place) {
-    std::vector<std::vector<const at::Tensor*>> ts(n_lists);
+    ts.resize(n_lists);
     same = n_lists > 0;
     for (size_t l = 0; l < n_lists; ++l) {
       if (!unpack(lists[l], ts[l])) return false;
@@ -148,6 +155,9 @@ struct Lists {
       meet = spans_meet(all, ends, in_place);
     }
     return true;
+  }
+  void mark_written(size_t l) const {
+    for (const at::Tensor* t : ts[l]) ::mark_written(*t);
   }
   bool usual(size_t l, bool f32) const {
     return (flags[l] & (kOtherDevice | kOtherDtype | kStrided | (f32 ? kNotF32 : 0))) == 0;
@@ -204,6 +214,16 @@ PyObject* overlap(PyObject*, PyObject* args) {
       ends.push_back(spans.size());
     }
     return PyBool_FromLong(spans_meet(spans, ends, in_place));
+  });
+}
+
+// written(list): what the Python layer's own calls wrote to.
+PyObject* written(PyObject*, PyObject* list) {
+  return guarded([&]() -> PyObject* {
+    std::vector<const at::Tensor*> ts;
+    if (!unpack(list, ts)) return nullptr;
+    for (const at::Tensor* t : ts) mark_written(*t);
+    Py_RETURN_NONE;
   });
 }
 
@@ -343,6 +363,7 @@ PyObject* score_rows_backward(PyObject*, PyObject* args) {
         rows.data_ptr(), rows.stride(0), dtype_code(rows.scalar_type()), R, (int)S, natural, stats, entropy,
         given ? reinterpret_cast<const long long*>(given->data_ptr()) : nullptr, n_given, gm, gg, ge, out.data_ptr(),
         out.stride(0), (void*)stream);
+    if (status == 0 && out_o != Py_None) mark_written(out);
     return Py_BuildValue("(iN)", status, out_o == Py_None ? wrap(out) : Py_NewRef(out_o));
   });
 }
@@ -380,6 +401,7 @@ PyObject* clip(PyObject*, PyObject* args) {
     const int status = reinterpret_cast<decltype(&kb_clip_gradients)>(fn)(
         src, write ? dst : nullptr, reinterpret_cast<const long long*>(x.counts.data()), x.dtypes[g].data(), (int)x.n, kind,
         max_norm, b.norm.data_ptr<float>(), b.ws.data_ptr(), bytes, (void*)stream);
+    if (status == 0 && write) x.mark_written(0);
     return Py_BuildValue("(iN)", status, wrap(b.norm));
   });
 }
@@ -406,6 +428,8 @@ PyObject* adam(PyObject*, PyObject* args) {
     const int status = reinterpret_cast<decltype(&kb_adam_step)>(fn)(
         at(0), at(3), at(1), at(2), reinterpret_cast<const long long*>(x.counts.data()), x.dtypes[3].data(), (int)x.n, lr,
         b1, b2, eps, wd, c1, c2, kind, max_norm, b.norm.data_ptr<float>(), b.ws.data_ptr(), bytes, (void*)stream);
+    if (status == 0)
+      for (size_t l = 0; l < 3; ++l) x.mark_written(l);
     return Py_BuildValue("(iN)", status, wrap(b.norm));
   });
 }
@@ -429,6 +453,7 @@ PyObject* fit_buffers(PyObject*, PyObject* args) {
 PyMethodDef kMethods[] = {
     {"gather", gather, METH_VARARGS, nullptr},
     {"overlap", overlap, METH_VARARGS, nullptr},
+    {"written", written, METH_O, nullptr},
     {"score_outputs", score_outputs, METH_VARARGS, nullptr},
     {"score_rows", score_rows, METH_VARARGS, nullptr},
     {"score_rows_backward", score_rows_backward, METH_VARARGS, nullptr},

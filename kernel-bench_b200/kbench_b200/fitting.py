@@ -10,7 +10,8 @@ counterpart of these kernels (the reference's fits run torch optimisers).
 
 Tensors are on one CUDA device; gradients are fp32, bf16 or fp16 (each its own), parameters and
 moments fp32.  Written tensors must each fill a block of memory (any order of dimensions) and share
-it with no other; gradients that are only read may have any strides.
+it with no other; gradients that are only read may have any strides.  What a call writes gets a new
+version, as after any in-place operation.
 """
 
 from __future__ import annotations
@@ -166,7 +167,9 @@ def clip_gradients(grads, max_norm, *, kind=2, out=None) -> torch.Tensor:
     if out is None:
         lists = _Lists(("grads",), (grads,), device, 1, False).apart()
         source = lists.described[0]
-        return _clip(source, source[0], lists.counts, len(grads), kind, max_norm, grads[0])
+        norm = _clip(source, source[0], lists.counts, len(grads), kind, max_norm, grads[0])
+        _lib.host().written(grads)
+        return norm
     lists = _Lists(("out", "grads"), (out, grads), device, 1, True)
     if lists.described[0][1] != lists.described[1][1]:
         raise RuntimeError("out must have the gradients' dtypes")
@@ -174,7 +177,9 @@ def clip_gradients(grads, max_norm, *, kind=2, out=None) -> torch.Tensor:
         grads = [_in_layout_of(g, o) for g, o in zip(grads, out)]
         lists = _Lists(("out", "grads"), (out, grads), device, 1, True)
     (destination, _), source = lists.apart().described[:2]
-    return _clip(source, destination, lists.counts, len(grads), kind, max_norm, grads[0])
+    norm = _clip(source, destination, lists.counts, len(grads), kind, max_norm, grads[0])
+    _lib.host().written(out)
+    return norm
 
 
 def adam_step(params, grads, exp_avg, exp_avg_sq, step: int, *, lr: float, beta1: float = 0.9, beta2: float = 0.999,
@@ -215,6 +220,8 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step: int, *, lr: float, beta1
     norm, ws = _lib.host().fit_buffers(params[0], size)
     _lib.call_on(device, "kb_adam_step", p, g, m, v, lists.counts, dtypes, len(grads), lr, beta1, beta2, eps,
                  weight_decay, correction1, correction2, kind, limit, norm.data_ptr(), ws.data_ptr(), size)
+    for tensors in (params, exp_avg, exp_avg_sq):
+        _lib.host().written(tensors)
     return None if max_norm is None else norm
 
 

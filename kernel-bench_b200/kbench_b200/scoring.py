@@ -150,6 +150,7 @@ def score_rows_backward(rows, stats, entropy, given=None, *, grad_log_mass=None,
     _lib.call_on(dev, "kb_score_rows_backward", rows.data_ptr(), rows.stride(0), _DTYPES[rows.dtype], R, S, natural,
                  stats.data_ptr(), _lib.ptr(entropy), _lib.ptr(columns), n_given, _lib.ptr(grad_log_mass),
                  _lib.ptr(grad_given), _lib.ptr(grad_entropy), out.data_ptr(), out.stride(0))
+    _lib.host().written([out])
     return out
 
 

@@ -121,3 +121,26 @@ def test_lists_are_described():
             host.gather(bad, 0, 0, False)
     with pytest.raises(TypeError):
         host.gather(ts, 0, 0, False)
+
+
+def test_written_tensors_get_a_new_version():
+    host = _host_or_skip()
+    a, b = torch.zeros(3), torch.zeros(4)
+    with torch.inference_mode():
+        c = torch.zeros(2)
+    host.written([a, c, b[1:]])  # a view's version is its base's; inference tensors have none
+    assert a._version == 1 and b._version == 1
+    with pytest.raises(TypeError):
+        host.written([a, None])
+
+
+def test_a_new_version_is_looked_at_again():
+    from types import SimpleNamespace
+
+    from kbench_b200 import glue
+    host = _host_or_skip()
+    static, w = SimpleNamespace(), torch.zeros(5)
+    assert glue.col_weights_uniform_for(static, w)
+    ctypes.c_float.from_address(w.data_ptr()).value = 1.0
+    host.written([w])
+    assert not glue.col_weights_uniform_for(static, w)

@@ -6,7 +6,7 @@ import sys
 import pytest
 import torch
 
-from kbench_b200 import fit, gen, runtime, scoring, tangent
+from kbench_b200 import fit, fitting, gen, runtime, scoring, tangent
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,24 @@ def test_command(cuda, capsys, monkeypatch):
     fit.main()
     got = json.loads(capsys.readouterr().out)
     assert got["objective_last"] < got["objective_first"] and len(got["origins"][0]["column"]) == 3
+
+
+def test_both_parameters_are_fitted(cuda):
+    """Uniform column weights that an update makes different: the next solves take them as they are."""
+    static, theta, cw = _problem(cuda, pi_iters=8, neumann_terms=8)
+    assert bool((cw == cw[0]).all())
+    opt = fitting.Adam([theta, cw], lr=0.05, max_norm=1.0)
+    for _ in range(2):
+        loss, saved = runtime.run_forward(static, theta, cw)
+        grads = runtime.run_backward(static, theta, cw, saved)
+        fresh = cw.clone()
+        want, wsaved = runtime.run_forward(static, theta, fresh)
+        wgrads = runtime.run_backward(static, theta, fresh, wsaved)
+        # the same solves, up to the order of fp32 additions
+        assert torch.allclose(loss, want, rtol=1e-6)
+        assert torch.allclose(saved["root_rows"], wsaved["root_rows"], rtol=1e-5, atol=1e-5)
+        for a, b in zip(grads, wgrads):
+            assert torch.allclose(a, b, rtol=1e-4, atol=1e-6)
+        runtime.run_forward(static, theta, cw)  # remembered once more for the tensor that is fitted
+        opt.step(grads)
+    assert not bool((cw == cw[0]).all())

@@ -459,3 +459,14 @@ def test_refusals(cuda):
     ):
         with pytest.raises(exc):
             call()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradient_buffer_gets_a_new_version(strided, cuda):
+    x = make_rows(5, 300, "solver", torch.float32, cuda)
+    rows = x.t().contiguous().t() if strided else x
+    s = scoring.score_rows(rows)
+    out = torch.empty_like(x)
+    before, kept = out._version, rows._version
+    assert scoring.score_rows_backward(rows, s.stats, None, grad_log_mass=s.log_mass, out=out) is out
+    assert out._version > before and rows._version == kept
