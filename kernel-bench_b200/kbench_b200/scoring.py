@@ -26,6 +26,7 @@ from . import _lib
 
 MAX_GIVEN = 32
 MAX_TOP = 32
+MAX_COLS = 1 << 30
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -55,6 +56,8 @@ def _check_rows(name: str, rows) -> torch.Tensor:
         raise RuntimeError(f"{name} supports fp32, bf16 and fp16 rows only (got {rows.dtype})")
     if rows.ndim != 2:
         raise ValueError(f"rows must be [R, S] (got {tuple(rows.shape)})")
+    if rows.shape[1] > MAX_COLS:  # the C entry point's length has 32 bits
+        raise ValueError(f"at most {MAX_COLS} columns (got {rows.shape[1]})")
     return rows if rows.stride(1) == 1 or rows.shape[1] <= 1 else rows.contiguous()
 
 
@@ -89,7 +92,7 @@ def _check_f32(name: str, t, shape, device):
 
 
 def score_rows(rows, given=None, *, top: int = 0, base=2) -> RowScores:
-    """Scores of ``rows`` [R, S] (fp32, bf16 or fp16; any row stride), without an autograd graph.
+    """Scores of ``rows`` [R, S <= 2^30] (fp32, bf16 or fp16; any row stride), without an autograd graph.
 
     ``given`` int64 or int32 [R] or [R, T <= 32]: the columns whose log probabilities are asked for;
     one outside [0, S) stands for none and scores 0.  ``top`` <= 32: how many of the largest entries

@@ -144,3 +144,15 @@ def test_a_new_version_is_looked_at_again():
     ctypes.c_float.from_address(w.data_ptr()).value = 1.0
     host.written([w])
     assert not glue.col_weights_uniform_for(static, w)
+
+
+def test_rows_past_the_longest_are_refused():
+    """Before a 32-bit argument can drop the upper bits of a row's length."""
+    from types import SimpleNamespace
+    for S in ((1 << 30) + 1, 1 << 32, (1 << 32) + 5):
+        rows = SimpleNamespace(device=SimpleNamespace(type="cuda"), dtype=torch.bfloat16, ndim=2, shape=(1, S),
+                               stride=lambda d: 1)
+        with pytest.raises(ValueError):
+            scoring._check_rows("score_rows", rows)
+    text = _lib.HEADER.read_text()
+    assert f"#define KB_MAX_SCORE_COLS {scoring.MAX_COLS}\n" in text

@@ -470,3 +470,12 @@ def test_gradient_buffer_gets_a_new_version(strided, cuda):
     before, kept = out._version, rows._version
     assert scoring.score_rows_backward(rows, s.stats, None, grad_log_mass=s.log_mass, out=out) is out
     assert out._version > before and rows._version == kept
+
+
+def test_rows_past_the_longest_are_refused(cuda):
+    x = torch.zeros((2, 1), dtype=torch.bfloat16, device=cuda)
+    for S in ((1 << 30) + 1, 1 << 32):
+        with pytest.raises(ValueError, match="columns"):
+            scoring.score_rows(x.expand(2, S))
+        with pytest.raises(ValueError, match="columns"):
+            scoring.score_rows_backward(x.expand(2, S), torch.zeros((2, 2), device=cuda), None)
