@@ -86,6 +86,11 @@ def host():
         except ImportError as e:
             raise RuntimeError(f"kbench_b200: _kb_host.so is not built (run kernel-bench_b200/kbench_b200/build.py): {e}") \
                 from e
+        from .build import host_target
+        target = getattr(_kb_host, "target", "an unknown torch")
+        if target != host_target():
+            raise RuntimeError(f"kbench_b200: _kb_host.so is built for {target}, not for {host_target()} "
+                               "(run kernel-bench_b200/kbench_b200/build.py)")
         _host = _kb_host
     return _host
 

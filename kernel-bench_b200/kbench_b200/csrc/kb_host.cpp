@@ -466,4 +466,11 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_kb_host", nullptr, -1, kMethods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__kb_host(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__kb_host(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddStringConstant(m, "target", KB_TARGET) != 0) {  // the Python and torch it is built for
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
