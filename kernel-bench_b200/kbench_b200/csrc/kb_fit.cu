@@ -313,7 +313,7 @@ struct AdamArgs {
 
 __device__ __forceinline__ void adam_entry(const AdamArgs& k, float g, float& p, float& m, float& v) {
   m = fmaf(k.one_minus_beta1, g, k.beta1 * m);
-  v = fmaf(k.one_minus_beta2, g * g, k.beta2 * v);
+  v = fmaf(k.one_minus_beta2 * g, g, k.beta2 * v);  // g * g is out of range from 1.8e19 on
   // the decay is a term of the update, not a factor 1 - lr wd, which fp32 holds to 6e-8 of 1:
   // 0.6 % of a decay of 1e-5
   p -= fmaf(k.decay, p, k.size * (m / fmaf(sqrtf(v), k.inv_root, k.eps)));
