@@ -272,10 +272,17 @@ __device__ __forceinline__ void gather_chunk(const Entry& e, long long k, int lo
   });
 }
 
+// The clip coefficient as head * tail: fp32 holds one below 2^-126 with few bits or not at all, and beside
+// entries of 1e38 the product is an ordinary number.  tail is 1, or 2^-64 for what is below 2^-100.
+struct Coef {
+  float head = 1.f, tail = 1.f;
+  __device__ __forceinline__ float operator*(float x) const { return (x * head) * tail; }
+};
+
 // The second pass reads the gradient for the last time and what else it moves but once: all of it is
 // marked to leave L2 first (ld.cs, st.cs), so that the gradient's end stays there until it is reached.
 template <typename T>
-__device__ __forceinline__ void clip_chunk(const Entry& e, long long k, int log2_chunk, float coef, int lane) {
+__device__ __forceinline__ void clip_chunk(const Entry& e, long long k, int log2_chunk, Coef coef, int lane) {
   constexpr int N = Vec<T>::N, U = 4;
   const T* p = static_cast<const T*>(e.p[0]);
   T* o = static_cast<T*>(e.p[1]);
@@ -292,7 +299,7 @@ __device__ __forceinline__ void clip_chunk(const Entry& e, long long k, int log2
         float f[N];
         Vec<T>::decode(q[u], f);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] *= coef;
+        for (int j = 0; j < N; ++j) f[j] = coef * f[j];
         __stcs(w + i + 32 * u, Vec<T>::encode(f));
       }
     }
@@ -302,7 +309,7 @@ __device__ __forceinline__ void clip_chunk(const Entry& e, long long k, int log2
     float f[N];
     load_vec(p, whole, i, m, f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] *= coef;
+    for (int j = 0; j < N; ++j) f[j] = coef * f[j];
     store_vec(o, whole, i, m, f);
   });
 }
@@ -320,7 +327,7 @@ __device__ __forceinline__ void adam_entry(const AdamArgs& k, float g, float& p,
 }
 
 template <typename T>
-__device__ __forceinline__ void adam_chunk(const Entry& e, long long k, int log2_chunk, float coef, const AdamArgs& a,
+__device__ __forceinline__ void adam_chunk(const Entry& e, long long k, int log2_chunk, Coef coef, const AdamArgs& a,
                                            int lane) {
   constexpr int N = Vec<T>::N;
   const T* gp = static_cast<const T*>(e.p[0]);
@@ -353,7 +360,7 @@ __device__ __forceinline__ void adam_chunk(const Entry& e, long long k, int log2
           Vec<float>::decode(mq[u * N / 4 + j], m);
           Vec<float>::decode(vq[u * N / 4 + j], v);
 #pragma unroll
-          for (int l = 0; l < 4; ++l) adam_entry(a, g[4 * j + l] * coef, p[l], m[l], v[l]);
+          for (int l = 0; l < 4; ++l) adam_entry(a, coef * g[4 * j + l], p[l], m[l], v[l]);
           __stcs(reinterpret_cast<uint4*>(pp + at) + j, Vec<float>::encode(p));
           __stcs(reinterpret_cast<uint4*>(mp + at) + j, Vec<float>::encode(m));
           __stcs(reinterpret_cast<uint4*>(vp + at) + j, Vec<float>::encode(v));
@@ -367,7 +374,7 @@ __device__ __forceinline__ void adam_chunk(const Entry& e, long long k, int log2
     load_vec(gp, whole, i, n, g);
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (j < n) adam_entry(a, g[j] * coef, pp[i + j], mp[i + j], vp[i + j]);
+      if (j < n) adam_entry(a, coef * g[j], pp[i + j], mp[i + j], vp[i + j]);
   });
 }
 
@@ -401,7 +408,7 @@ __device__ __forceinline__ double gather_share(const Table& t, Share w, bool squ
 
 // Backwards, so that what the norm's pass read last comes first.
 template <bool ADAM>
-__device__ __forceinline__ void apply_share(const Table& t, Share w, float coef, const AdamArgs& a, int lane) {
+__device__ __forceinline__ void apply_share(const Table& t, Share w, Coef coef, const AdamArgs& a, int lane) {
   if (w.w >= t.n_chunks) return;
   const Entry* e = entries(t);
   int at = -1;
@@ -436,9 +443,11 @@ __device__ __forceinline__ double block_join(double v, bool square, double* scra
   return r;
 }
 
-__device__ __forceinline__ float clip_coefficient(double norm, double max_norm) {
+__device__ __forceinline__ Coef clip_coefficient(double norm, double max_norm) {
   const double c = max_norm / (norm + (double)kClipEps);
-  return c >= 1.0 ? 1.f : (float)c;  // a NaN stays
+  if (c >= 1.0) return Coef{};
+  if (c < 0x1p-100) return Coef{(float)(c * 0x1p64), 0x1p-64f};
+  return Coef{(float)c, 1.f};  // a NaN stays
 }
 
 struct Step {
@@ -461,7 +470,7 @@ template <bool ADAM>
 __global__ void __launch_bounds__(kThreads, 3) apply_kernel(const __grid_constant__ Table t, const Step s,
                                                           const double* partials, int n_partials) {
   __shared__ double scratch[kThreads / 32];
-  float coef = 1.f;
+  Coef coef;
   if (s.clip) {  // every CTA joins the partials itself, in the same order
     double v = 0.0;
     for (int i = threadIdx.x; i < n_partials; i += kThreads) v = s.square ? v + partials[i] : max_nan(v, partials[i]);
@@ -486,7 +495,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_kernel(const __gri
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
   const Share r{cta * (kClusterThreads / 32) + wid, n_ctas * (kClusterThreads / 32)};
-  float coef = 1.f;
+  Coef coef;
   if (s.clip) {
     double v = block_join(gather_share(t, r, s.square, lane), s.square, scratch);
     if (n_ctas > 1) {
