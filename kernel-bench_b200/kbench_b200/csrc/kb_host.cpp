@@ -5,13 +5,13 @@
 // which the Python layer then refuses, copies or calls itself (a score_rows of one row 15 us of host
 // time by way of Python, 10 here).
 #include <ATen/ATen.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "kb_solver.h"
 
 #include <algorithm>
 #include <cstdint>
-#include <exception>
 #include <vector>
 
 namespace {
@@ -41,14 +41,12 @@ bool unpack(PyObject* seq, std::vector<const at::Tensor*>& out) {
   return true;
 }
 
+// With torch's exceptions as the Python ones they stand for (the allocator's: torch.OutOfMemoryError).
 template <typename F>
 PyObject* guarded(const F& f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
 }
 
 // What a kernel wrote to through its address counts as changed in place: the version by which autograd and

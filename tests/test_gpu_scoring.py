@@ -479,3 +479,11 @@ def test_rows_past_the_longest_are_refused(cuda):
             scoring.score_rows(x.expand(2, S))
         with pytest.raises(ValueError, match="columns"):
             scoring.score_rows_backward(x.expand(2, S), torch.zeros((2, 2), device=cuda), None)
+
+
+def test_outputs_that_do_not_fit_are_out_of_memory(cuda):
+    """The allocator's own exception, with nothing launched: 205 GB of alternatives."""
+    rows = torch.zeros((1, 4), device=cuda).expand(1_600_000_000, 4)
+    with pytest.raises(torch.OutOfMemoryError):
+        scoring.score_rows(rows, top=32)
+    torch.cuda.empty_cache()
