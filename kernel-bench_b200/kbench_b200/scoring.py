@@ -98,9 +98,10 @@ def score_rows(rows, given=None, *, top: int = 0, base=2) -> RowScores:
     one outside [0, S) stands for none and scores 0.  ``top`` <= 32: how many of the largest entries
     are listed (equal entries by the lower column)."""
     top = int(top)
-    out = _lib.call_host("score_rows", "kb_score_rows", rows.device, rows, given, top, _natural(base))
-    if out is not None:
-        return RowScores(*out)
+    if 0 <= top <= MAX_TOP:  # the extension takes a C int
+        out = _lib.call_host("score_rows", "kb_score_rows", rows.device, rows, given, top, _natural(base))
+        if out is not None:
+            return RowScores(*out)
     rows = _check_rows("score_rows", rows)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be in [0, {MAX_TOP}] (got {top})")

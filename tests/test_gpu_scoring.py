@@ -487,3 +487,10 @@ def test_outputs_that_do_not_fit_are_out_of_memory(cuda):
     with pytest.raises(torch.OutOfMemoryError):
         scoring.score_rows(rows, top=32)
     torch.cuda.empty_cache()
+
+
+def test_tops_past_an_integer_are_refused(cuda):
+    x = torch.zeros((4, 9), device=cuda)
+    for top in (1 << 31, -(1 << 40)):
+        with pytest.raises(ValueError):
+            scoring.score_rows(x, top=top)
