@@ -122,7 +122,8 @@ def score_rows_backward(rows, stats, entropy, given=None, *, grad_log_mass=None,
     ``stats`` [R, 2] and ``entropy`` [R] (needed with ``grad_entropy`` alone) are the forward's;
     ``grad_log_mass`` [R], ``grad_given`` (shaped as ``given``) and ``grad_entropy`` [R] the cotangents
     (``None``: zero).  To differentiate listed alternatives pass their columns as ``given``.  The
-    gradient is 0 at impossible columns.  ``out``: a buffer [R, S] to write to (not ``rows``)."""
+    gradient is 0 at impossible columns.  ``out``: a buffer [R, S] to write to, whose address range does not
+    meet that of ``rows``."""
     natural = _natural(base)
     got = _lib.call_host("score_rows_backward", "kb_score_rows_backward", rows.device, rows, stats, entropy, given,
                          grad_log_mass, grad_given, grad_entropy, natural, out)
@@ -149,7 +150,7 @@ def score_rows_backward(rows, stats, entropy, given=None, *, grad_log_mass=None,
         raise RuntimeError("out must have the rows' device and dtype")
     elif out.shape != rows.shape or (S > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < S):
         raise ValueError("out must be [R, S] with unit column stride and rows that do not overlap")
-    elif out.untyped_storage().data_ptr() == rows.untyped_storage().data_ptr() and _overlap(out, rows):
+    elif _overlap(out, rows):
         raise ValueError("out must not overlap rows")
     _lib.call_on(dev, "kb_score_rows_backward", rows.data_ptr(), rows.stride(0), _DTYPES[rows.dtype], R, S, natural,
                  stats.data_ptr(), _lib.ptr(entropy), _lib.ptr(columns), n_given, _lib.ptr(grad_log_mass),
@@ -159,7 +160,8 @@ def score_rows_backward(rows, stats, entropy, given=None, *, grad_log_mass=None,
 
 
 def _overlap(a, b) -> bool:
-    """Whether the address ranges of two row matrices meet."""
+    """Whether the address ranges of two row matrices meet (storages do not tell: one imported by another
+    library's view of the same memory starts elsewhere)."""
     def span(t):
         if t.numel() == 0:
             return 0, 0

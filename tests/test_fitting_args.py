@@ -156,3 +156,11 @@ def test_rows_past_the_longest_are_refused():
             scoring._check_rows("score_rows", rows)
     text = _lib.HEADER.read_text()
     assert f"#define KB_MAX_SCORE_COLS {scoring.MAX_COLS}\n" in text
+
+
+def test_shared_memory_is_seen_through_other_storages():
+    flat = torch.zeros(100)
+    rows = flat[:60].view(6, 10)
+    same = torch.from_dlpack(flat[30:90]).view(6, 10)
+    assert same.untyped_storage().data_ptr() != rows.untyped_storage().data_ptr()
+    assert scoring._overlap(same, rows) and not scoring._overlap(torch.from_dlpack(flat[60:]).view(4, 10), rows)

@@ -494,3 +494,14 @@ def test_tops_past_an_integer_are_refused(cuda):
     for top in (1 << 31, -(1 << 40)):
         with pytest.raises(ValueError):
             scoring.score_rows(x, top=top)
+
+
+def test_output_on_the_rows_through_another_storage_is_refused(cuda):
+    flat = torch.zeros(100, device=cuda)
+    rows = flat[:60].view(6, 10)
+    s = scoring.score_rows(rows)
+    for at in (0, 30):
+        out = torch.from_dlpack(flat[at:at + 60]).view(6, 10)
+        with pytest.raises(ValueError):
+            scoring.score_rows_backward(rows, s.stats, None, grad_log_mass=s.log_mass, out=out)
+    assert not bool(flat.any())
