@@ -799,7 +799,8 @@ struct ScoreGradArgs {
 // dL/dx_s = p_s (a - sum_t g_t - h ln2 (z_s - log2 Sigma + H)) + sum_{t: given_t = s} g_t, with the
 // cotangents a of log_mass, g of the given columns and h of the entropy, H in bits (the factor
 // ln u of d log_u and the one of d u^x cancel, so both bases share it).  Impossible columns are
-// constants: no gradient at them, none through a given column that is one.
+// constants: no gradient at them, none through a given column that is one.  That holds beside cotangents
+// that are not finite too (functions of an empty row's log mass, -inf, have such).
 struct Gradient {
   float m, scale, direct, bend;
   __device__ __forceinline__ Gradient(const ScoreGradArgs& a, long long r, float m_row, float sum, float g_all) {
@@ -812,6 +813,12 @@ struct Gradient {
     // p (base - h (z + bits)) = 2^z direct - 2^z z bend
     direct = ((a.g_mass ? a.g_mass[r] : 0.f) - g_all - h * bits) * inv;
     bend = h * inv;
+    if (empty) direct = bend = 0.f;
+  }
+  // Whether the row is a distribution (else its stats are NaN) beside which a factor is not finite: 0 times it
+  // is NaN at the impossible columns.
+  __device__ __forceinline__ bool odd() const {
+    return m == m && !(fabsf(direct) + fabsf(bend) < __int_as_float(0x7f800000));
   }
   // without the given columns' own terms
   __device__ __forceinline__ float operator()(float x) const {
@@ -882,6 +889,11 @@ __global__ void __launch_bounds__(32 * kWarps, 4) score_rows_backward_kernel(con
       }
     }
   }
+  if (gradient.odd()) {
+    __syncwarp();  // after the stores above
+    for (int col = max(0, row.column(b0, 0, 0)) + lane; col < min(row.S, row.column(b1, 0, 0)); col += 32)
+      if (is_neg_inf(Vec<T>::up(x[col]))) out[col] = Vec<T>::down(0.f);
+  }
   if (a.n_given == 0) return;
   // equal columns are added up by the first lane that has one, in the lanes' order
   float add = 0.f;
@@ -926,9 +938,11 @@ __global__ void __launch_bounds__(32 * kWarps) score_short_backward_kernel(const
       if (i * G + lane == (int)t) add[i] += g;
   }
   const Gradient gradient(a, r, m_row, sum, g_all);
+  const bool odd = gradient.odd();
 #pragma unroll
   for (int i = 0; i < E; ++i)
-    if (i * G + lane < S) out[i * G + lane] = Vec<T>::down(gradient(f[i]) + add[i]);
+    if (i * G + lane < S)
+      out[i * G + lane] = Vec<T>::down(odd && is_neg_inf(f[i]) ? 0.f : gradient(f[i]) + add[i]);
 }
 
 template <typename T>

@@ -505,3 +505,30 @@ def test_output_on_the_rows_through_another_storage_is_refused(cuda):
         with pytest.raises(ValueError):
             scoring.score_rows_backward(rows, s.stats, None, grad_log_mass=s.log_mass, out=out)
     assert not bool(flat.any())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("S", [5, 63, 100, 250, 700, 4099])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_impossible_columns_keep_zero_beside_any_cotangent(S, dtype, bad, cuda):
+    """Rows of -inf alone have log mass -inf, whose functions have cotangents that are not finite."""
+    x = make_rows(6, S, "plain", DTYPES[dtype], cuda)
+    x[1], x[4] = -math.inf, -math.inf
+    x[2, ::2], x[3, 1:] = -math.inf, -math.inf
+    given = torch.zeros((6, 2), dtype=torch.int64, device=cuda)
+    given[:, 1] = S // 2
+    s = scoring.score_rows(x, given)
+    one = torch.ones(6, device=cuda)
+    cot = one.clone()
+    cot[[1, 2, 4]] = bad
+    for k in ("grad_log_mass", "grad_entropy", "grad_given"):
+        got = scoring.score_rows_backward(x, s.stats, s.entropy, given, **{k: cot[:, None].repeat(1, 2) if k == "grad_given" else cot})
+        assert bool((got[torch.isneginf(x)] == 0).all()), k
+        want = scoring.score_rows_backward(x, s.stats, s.entropy, given, **{k: one[:, None].repeat(1, 2) if k == "grad_given" else one})
+        for r in (0, 3, 5):
+            assert torch.equal(got[r], want[r])
+        # the possible columns of row 2 follow the formula: a cotangent at impossible given columns does not count
+        live = got[2][~torch.isneginf(x[2])]
+        counts = k != "grad_given" or bool((x[2, given[2]] > -math.inf).any())
+        if live.numel() > 2:
+            assert bool(torch.isfinite(live).all()) != counts
