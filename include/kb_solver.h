@@ -627,7 +627,8 @@ int kb_plan_build(long long n_rows, long long n_splits, int n_waves, const long 
  *   (0 for one outside [0,n_cols)), top_log_prob / top_column int64 [n_rows,n_top]: the largest
  *   entries in order, equal ones by the lower column; -inf and -1 past n_cols.
  * A row of -inf alone: log_mass and log probabilities -inf, entropy 0, stats (-inf, 0).  A row
- * with NaN or +inf: NaN throughout, top columns -1.  Outputs are fp32, contiguous. */
+ * with NaN or +inf: NaN throughout, top columns -1.  Outputs are fp32, contiguous.  Here and below an
+ * address off its type's boundary is KB_ERR_ARG. */
 #define KB_MAX_GIVEN 32
 #define KB_MAX_TOP 32
 #define KB_MAX_SCORE_COLS 1073741824

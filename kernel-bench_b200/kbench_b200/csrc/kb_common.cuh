@@ -19,6 +19,9 @@
 namespace kb {
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+// Whether an address can be used for items of so many bytes (NULL can): one off their boundary faults.
+inline bool on_boundary(const void* p, unsigned bytes) { return (reinterpret_cast<unsigned long long>(p) & (bytes - 1)) == 0; }
+
 __device__ __forceinline__ bool is_neg_inf(float x) { return x == __int_as_float(0xff800000); }
 __device__ __forceinline__ float safe_max(float m) { return is_neg_inf(m) ? 0.0f : m; }
 

@@ -643,7 +643,8 @@ extern "C" int kb_clip_gradients(const long long* grads, const long long* outs, 
                                  const int* dtypes, int n_tensors, int kind, double max_norm, float* norm_out,
                                  void* ws, long long ws_bytes, void* stream) {
   if (n_tensors < 0 || (kind != 0 && kind != 2) || !norm_out || !ws || ws_bytes < workspace_bytes(n_tensors) ||
-      (n_tensors > 0 && (!grads || !counts || !dtypes)) || (outs && !(max_norm >= 0.0)))
+      (n_tensors > 0 && (!grads || !counts || !dtypes)) || (outs && !(max_norm >= 0.0)) ||
+      !on_boundary(ws, 16) || !on_boundary(norm_out, 4))
     return KB_ERR_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
   Table t{};
@@ -661,7 +662,8 @@ extern "C" int kb_adam_step(const long long* params, const long long* grads, con
                             void* ws, long long ws_bytes, void* stream) {
   if (n_tensors < 0 || (kind != -1 && kind != 0 && kind != 2) || !ws || ws_bytes < workspace_bytes(n_tensors) ||
       (kind >= 0 && (!norm_out || !(max_norm >= 0.0))) || !(correction1 > 0.0) || !(correction2 > 0.0) ||
-      (n_tensors > 0 && (!params || !grads || !exp_avg || !exp_avg_sq || !counts || !grad_dtypes)))
+      (n_tensors > 0 && (!params || !grads || !exp_avg || !exp_avg_sq || !counts || !grad_dtypes)) ||
+      !on_boundary(ws, 16) || !on_boundary(norm_out, 4))
     return KB_ERR_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
   Table t{};

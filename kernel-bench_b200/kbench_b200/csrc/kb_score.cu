@@ -25,6 +25,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "kb_common.cuh"
 #include "kb_solver.h"
 
@@ -1029,6 +1031,12 @@ cudaError_t launch_scores_of(const ScoreArgs& a, bool natural, cudaStream_t st) 
 
 }  // namespace
 
+static bool floats_on_boundary(std::initializer_list<const float*> ps) {
+  for (const float* p : ps)
+    if (!kb::on_boundary(p, 4)) return false;
+  return true;
+}
+
 extern "C" int kb_score_rows(const void* rows, long long row_stride, int dtype, long long n_rows, int n_cols,
                              int natural, const long long* given, int n_given, int n_top, float* log_mass,
                              float* entropy, float* given_log_prob, float* top_log_prob, long long* top_column,
@@ -1039,6 +1047,9 @@ extern "C" int kb_score_rows(const void* rows, long long row_stride, int dtype, 
   if (n_rows == 0) return KB_OK;
   if ((!rows && n_cols > 0) || !log_mass || !entropy || !stats || (n_given > 0 && (!given || !given_log_prob)) ||
       (n_top > 0 && (!top_log_prob || !top_column)))
+    return KB_ERR_ARG;
+  if (!on_boundary(rows, dtype == 0 ? 4 : 2) || !on_boundary(given, 8) || !on_boundary(top_column, 8) ||
+      !floats_on_boundary({log_mass, entropy, given_log_prob, top_log_prob, stats}))
     return KB_ERR_ARG;
   if (n_rows > 0x7fffffffll || n_cols > KB_MAX_SCORE_COLS) return KB_ERR_SIZE;
   ScoreArgs a{rows, row_stride, n_rows, n_cols, n_given, n_top, natural ? kLog2e : 1.f, natural ? kLn2 : 1.f,
@@ -1061,6 +1072,10 @@ extern "C" int kb_score_rows_backward(const void* rows, long long row_stride, in
   if (n_rows == 0 || n_cols == 0) return KB_OK;
   if (!rows || !grad_rows || !stats || (grad_entropy && !entropy) || (n_given > 0 && grad_given && !given) ||
       (n_rows > 1 && grad_stride < n_cols))
+    return KB_ERR_ARG;
+  const unsigned width = dtype == 0 ? 4 : 2;
+  if (!on_boundary(rows, width) || !on_boundary(grad_rows, width) || !on_boundary(given, 8) ||
+      !floats_on_boundary({stats, entropy, grad_log_mass, grad_given, grad_entropy}))
     return KB_ERR_ARG;
   if (n_rows > 0x7fffffffll || n_cols > KB_MAX_SCORE_COLS) return KB_ERR_SIZE;
   ScoreGradArgs a{rows, row_stride, n_rows, n_cols, grad_given ? n_given : 0, natural ? kLog2e : 1.f, stats, entropy,

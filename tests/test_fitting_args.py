@@ -164,3 +164,29 @@ def test_shared_memory_is_seen_through_other_storages():
     same = torch.from_dlpack(flat[30:90]).view(6, 10)
     assert same.untyped_storage().data_ptr() != rows.untyped_storage().data_ptr()
     assert scoring._overlap(same, rows) and not scoring._overlap(torch.from_dlpack(flat[60:]).view(4, 10), rows)
+
+
+def test_addresses_off_their_types_boundary_are_refused():
+    """Such an access would fault on the device."""
+    lib = _lib_or_skip()
+    p = {"rows": 4096, "given": 4096, "mass": 4096, "entropy": 4096, "glp": 4096, "tlp": 4096, "tcol": 4096, "stats": 4096}
+    for dtype, off in ((0, {"rows": 4098}), (1, {"rows": 4097}), (2, {"rows": 4099}), (0, {"given": 4100}),
+                       (0, {"mass": 4098}), (0, {"entropy": 4097}), (0, {"glp": 4098}), (0, {"tlp": 4098}),
+                       (0, {"tcol": 4100}), (0, {"stats": 4098})):
+        a = dict(p, **off)
+        assert lib.kb_score_rows(a["rows"], 8, dtype, 2, 8, 0, a["given"], 1, 1, a["mass"], a["entropy"], a["glp"],
+                                 a["tlp"], a["tcol"], a["stats"], None) == _lib.KB_ERR_ARG, off
+    p = {"rows": 4096, "stats": 4096, "entropy": 4096, "given": 4096, "gm": 4096, "gg": 4096, "ge": 4096, "out": 8192}
+    for dtype, off in ((0, {"rows": 4098}), (1, {"rows": 4097}), (1, {"out": 8193}), (0, {"out": 8194}), (0, {"given": 4100}),
+                       (0, {"stats": 4098}), (0, {"entropy": 4098}), (0, {"gm": 4098}), (0, {"gg": 4098}), (0, {"ge": 4098})):
+        a = dict(p, **off)
+        assert lib.kb_score_rows_backward(a["rows"], 8, dtype, 2, 8, 0, a["stats"], a["entropy"], a["given"], 1, a["gm"],
+                                          a["gg"], a["ge"], a["out"], 8, None) == _lib.KB_ERR_ARG, off
+    size = ctypes.c_longlong()
+    lib.kb_fit_workspace(1, ctypes.byref(size))
+    one, dtypes = (ctypes.c_longlong * 1), (ctypes.c_int * 1)(0)
+    for ws, norm in ((4104, 4096), (4096, 4098)):
+        assert lib.kb_clip_gradients(one(4096), one(4096), one(4), dtypes, 1, 2, 1.0, norm, ws, size.value,
+                                     None) == _lib.KB_ERR_ARG
+        assert lib.kb_adam_step(one(4096), one(4096), one(4096), one(4096), one(4), dtypes, 1, 0.1, 0.9, 0.9, 1e-8, 0.0, 0.1,
+                                0.1, 2, 1.0, norm, ws, size.value, None) == _lib.KB_ERR_ARG
