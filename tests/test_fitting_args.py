@@ -190,3 +190,9 @@ def test_addresses_off_their_types_boundary_are_refused():
                                      None) == _lib.KB_ERR_ARG
         assert lib.kb_adam_step(one(4096), one(4096), one(4096), one(4096), one(4), dtypes, 1, 0.1, 0.9, 0.9, 1e-8, 0.0, 0.1,
                                 0.1, 2, 1.0, norm, ws, size.value, None) == _lib.KB_ERR_ARG
+
+
+def test_strides_of_dimensions_of_one_do_not_matter():
+    a = torch.zeros(5 * 3).as_strided((3, 1, 5), (1, 99, 3))
+    b = torch.zeros(5 * 3).as_strided((3, 1, 5), (1, 15, 3))
+    assert fitting._dense(a) and fitting._same_layout(a, b) and not fitting._same_layout(a, torch.zeros(3, 1, 5))
