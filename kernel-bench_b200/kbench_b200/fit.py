@@ -74,11 +74,12 @@ def main():
     observed = None if a.origin is None else torch.full_like(roots, a.origin, dtype=torch.int64)
     r = fit_rates(static, theta, cw, steps=a.steps, lr=a.lr, max_norm=a.max_norm, observed=observed, top=a.top)
     s = r.scores
+    columns, probs = ([[]] * len(s.entropy) if t is None else t.tolist() for t in (s.top_column, s.top_log_prob))
     print(json.dumps({
         "objective_first": float(r.objective[0]), "objective_last": float(r.objective[-1]),
         "grad_norm_last": float(r.grad_norm[-1]),
         "origins": [{"column": c, "log2_prob": [round(v, 4) for v in p], "entropy_bits": round(h, 4)} for c, p, h in
-                    list(zip(s.top_column.tolist(), s.top_log_prob.tolist(), s.entropy.tolist()))[:8]]}))
+                    list(zip(columns, probs, s.entropy.tolist()))[:8]]}))
 
 
 if __name__ == "__main__":

@@ -137,3 +137,11 @@ def test_both_parameters_are_fitted(cuda):
         runtime.run_forward(static, theta, cw)  # remembered once more for the tensor that is fitted
         opt.step(grads)
     assert not bool((cw == cw[0]).all())
+
+
+def test_command_without_alternatives(cuda, capsys, monkeypatch):
+    monkeypatch.setattr(sys, "argv", ["fit", "--config", "1", "--steps", "2", "--top", "0"])
+    fit.main()
+    got = json.loads(capsys.readouterr().out)
+    assert got["origins"] and all(o["column"] == [] and o["log2_prob"] == [] and o["entropy_bits"] >= 0
+                                  for o in got["origins"])
