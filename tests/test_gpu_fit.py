@@ -1,6 +1,7 @@
 """The fit of theta (``kbench_b200.fit``) and the root rows' cotangent of the backward solve."""
 
 import json
+import math
 import sys
 
 import pytest
@@ -145,3 +146,35 @@ def test_command_without_alternatives(cuda, capsys, monkeypatch):
     got = json.loads(capsys.readouterr().out)
     assert got["origins"] and all(o["column"] == [] and o["log2_prob"] == [] and o["entropy_bits"] >= 0
                                   for o in got["origins"])
+
+
+@pytest.mark.parametrize("engine", ["fused", "wrappers"])
+def test_the_losss_own_cotangent_by_value(engine, cuda):
+    """The cotangents of +- log mass change the gradient by +- that of the root rows' log mass, which the
+    tangent solver gives along any direction (to the acceptance of a tangent, as above); with + the seed
+    is zero and only the extinction vector's term is left, with - the root part doubles."""
+    static, theta, cw = _problem(cuda, engine)
+    _, saved = runtime.run_forward(static, theta, cw)
+    rows = saved["root_rows"]
+    s = scoring.score_rows(rows)
+    cot = scoring.score_rows_backward(rows, s.stats, None, grad_log_mass=torch.ones_like(s.log_mass))
+    base = runtime.run_backward(static, theta, cw, saved)[0].double()
+    up, down = (runtime.run_backward(static, theta, cw, saved, root_cotangent=sign * cot)[0].double() - base
+                for sign in (1.0, -1.0))
+    fused, ft, fc = _problem(cuda)
+    _, fsaved = runtime.run_forward(fused, ft, fc)
+    V = torch.randn((6, *theta.shape), generator=torch.Generator().manual_seed(2)).to(cuda)
+    V[0] = theta.sign() + 2.0  # all entries of one sign: the terms add up
+    V[1] = 1.0
+    wants = []
+    for v, dr in zip(V, tangent.jvp_batch(fused, ft, V, fsaved)):
+        want = float((torch.softmax(fsaved["root_rows"].double() * math.log(2.0), 1) * dr.double()).sum())
+        for sign, change in ((1.0, up), (-1.0, down)):
+            terms = v.double() * change
+            assert abs(sign * float(terms.sum()) - want) <= 1e-3 * float(terms.abs().sum())
+        wants.append(abs(want))
+    assert min(wants) > 0.0
+    # a zero seed: what is left does not depend on the root rows at all
+    zero = runtime.run_backward(static, theta, cw, saved, root_cotangent=cot)[0].double()
+    twice = runtime.run_backward(static, theta, cw, saved, root_cotangent=cot * 2.0)[0].double()
+    assert float((twice - zero - up).norm()) <= 1e-3 * float(up.norm())
