@@ -532,3 +532,41 @@ def test_impossible_columns_keep_zero_beside_any_cotangent(S, dtype, bad, cuda):
         counts = k != "grad_given" or bool((x[2, given[2]] > -math.inf).any())
         if live.numel() > 2:
             assert bool(torch.isfinite(live).all()) != counts
+
+
+# ---- every form of the kernels -----------------------------------------------------------------
+
+# rows past 1,024 columns: a warp a row with two batches under way (the first three) and one; four warps a row;
+# eight, some of them without a batch in 16 bits; a CTA a row of many
+FORMS = [(3, 1400), (1000, 4095), (2300, 5001), (2500, 4095), (500, 8191), (800, 5003), (400, 5003), (1000, 24001)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", FORMS)
+@pytest.mark.parametrize("kind,base", [("solver", 2), ("plain", "e"), ("masked", 2), ("masked", "e"), ("ties", 2), ("one", 2)])
+def test_forms(shape, dtype, kind, base, cuda):
+    x = make_rows(*shape, kind, DTYPES[dtype], cuda, seed=4)
+    given = make_given(*shape, 2, cuda)
+    ref = None
+    for top in (0, 1, 8, 32):
+        s = scoring.score_rows(x, given, top=top, base=base)
+        if ref is None:
+            check_scores(s, x, given, 0, base)
+            wide = scoring.score_rows(x, given, top=32, base=base)
+            check_scores(wide, x, given, 32, base)
+            ref = wide
+        else:  # the same row sums, and the head of the same list
+            for a, b in zip((s.log_mass, s.entropy, s.given_log_prob, s.stats, s.top_log_prob, s.top_column),
+                            (ref.log_mass, ref.entropy, ref.given_log_prob, ref.stats, ref.top_log_prob[:, :top],
+                             ref.top_column[:, :top])):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", [(3, 1400), (5000, 257), (5000, 1023), (5000, 4095), (500, 8191), (2500, 9001)])
+@pytest.mark.parametrize("kind,base", [("solver", 2), ("plain", "e"), ("masked", 2), ("masked", "e")])
+def test_gradient_forms(shape, dtype, kind, base, cuda):
+    x = make_rows(*shape, kind, DTYPES[dtype], cuda, seed=6)
+    given = make_given(*shape, 3, cuda)
+    given[:, 2] = given[:, 0]
+    check_grad(x, given, base, scoring.score_rows(x, given, base=base))
