@@ -188,7 +188,11 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, step: int, *, lr: float, beta1
               eps: float = 1e-8, weight_decay: float = 0.0, max_norm=None, kind=2):
     """Adam's update number ``step`` (from 1) of ``params`` and the moments in place, with decoupled
     weight decay; with ``max_norm`` the gradients count as clipped by their global norm, which is
-    returned (a device scalar; ``None`` without).  ``grads`` are not changed."""
+    returned (a device scalar; ``None`` without).  ``grads`` are not changed.
+
+    The bias corrections of ``step`` are taken on the host: a captured call replays that step's, whatever
+    the replay's number, so capture one only where they no longer change (late steps).  As with any graph,
+    a replay gives the written tensors no new version."""
     step = int(step)
     if step < 1:
         raise ValueError(f"step counts from 1 (got {step})")

@@ -570,3 +570,21 @@ def test_gradient_forms(shape, dtype, kind, base, cuda):
     given = make_given(*shape, 3, cuda)
     given[:, 2] = given[:, 0]
     check_grad(x, given, base, scoring.score_rows(x, given, base=base))
+
+
+@pytest.mark.parametrize("shape", [(40, 63), (40, 1023)])
+def test_gradient_graph_capture(shape, cuda):
+    x = make_rows(*shape, "solver", torch.float32, cuda)
+    given = make_given(*shape, 2, cuda)
+    a, g, h = cotangents(shape[0], 2, cuda)
+
+    def step():
+        s = scoring.score_rows(x, given)
+        return scoring.score_rows_backward(x, s.stats, s.entropy, given, grad_log_mass=a, grad_given=g, grad_entropy=h)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.copy_(make_rows(*shape, "solver", torch.float32, cuda, seed=9))
+    graph.replay()
+    assert torch.equal(got, step())
