@@ -18,8 +18,10 @@
 // one cluster, whose CTAs join their sums over distributed shared memory, in one launch (one family of
 // 1,023 columns 5 us).  Else a first kernel leaves a partial sum a CTA, and the second, whose CTAs each
 // join them, goes through every warp's chunks backwards, from what the first left in L2.
-// Measured: 201 M bf16 entries 66 + 127 us, 6.1 and 6.3 TB/s (93 and 97 % of the copy bandwidth);
-// Adam over 104 M fp32 entries 70 + 500 us, 5.9 and 5.8 TB/s (90 and 89 %).
+// Measured, call after call: 201 M bf16 entries 81 + 124 us, 5.0 and 6.5 TB/s (76 and 99 % of the copy
+// bandwidth); Adam over 104 M fp32 entries 83 + 507 us, 5.0 and 5.7 TB/s (76 and 87 %), with bf16 gradients 45 + 540
+// us (4.6 and 5.0 TB/s).  The norm's pass also writes back what the call before left dirty in L2: with L2 flushed it
+// takes 64, 69 and 39 us (6.3, 6.0 and 5.3 TB/s).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,8 +37,8 @@ constexpr float kClipEps = 1e-6f;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kThreads = 256;
 // CTAs of the norm kernel and of the second one, all resident: more bytes under way help a kernel that
-// only reads, and fewer streams one that also writes (201 M bf16: norm 66 us with 5 an SM, 72 with 8;
-// clip 127 with 3, 137 with 2; Adam 104 M: 500 us with 3, 514 with 4).
+// only reads, and fewer streams one that also writes (with L2 flushed, 201 M bf16: norm 66 us with 5 an SM, 72
+// with 8; clip 127 with 3, 137 with 2; Adam 104 M: 500 us with 3, 514 with 4).
 constexpr int kNormCtas = 148 * 5;
 constexpr int kApplyCtas = 148 * 3;
 constexpr int kClusterThreads = 512;  // a CTA of the one-cluster form

@@ -196,7 +196,8 @@ PyObject* gather(PyObject*, PyObject* args) {
   });
 }
 
-// overlap(written, read, in_place): gather's `meet` alone, of tensors on any device.
+// overlap(written, read, in_place): gather's `meet` alone, of tensors on any device, so that the search can be tested
+// without a GPU.
 PyObject* overlap(PyObject*, PyObject* args) {
   PyObject *a, *b;
   int in_place;

@@ -656,7 +656,8 @@ __global__ void __launch_bounds__(32 * kWarps) score_short_kernel(const ScoreArg
 // warps 462, and 610 with the next row asked into L2 by bulk prefetches).  More rows under way help
 // too: at 64 registers (32 warps an SM) 367 us where 76 (24 warps) take 411.  16-bit rows, whose
 // batches hold twice the entries, are bound by their instructions and keep 80.
-// Measured: 128,282 x 4,095 fp32 with 8 columns 362 us, 5.8 TB/s, 89 % of the copy bandwidth.
+// Measured: 128,282 x 4,095 fp32 with 8 columns 354 us, 6.0 TB/s, 91 % of the copy bandwidth; after a second of
+// nothing else, at 1.6 GHz under the power cap, 390 us a call, 5.4 TB/s, 83 %.
 // Where all rows are under way at once the warps are too few to fill memory with one batch each; with
 // AHEAD = 2 they ask for two (2,300 x 32,001 fp32: 76 us, 82 with one; 1,700 x 4,095: 16 and 18).
 template <typename T, bool TOP, bool NATURAL, int AHEAD>
@@ -830,7 +831,7 @@ struct Gradient {
 };
 
 // A warp takes `chunk` batches of a row: one read and one write of each entry, so memory bounds it
-// (32,071 x 4,095 fp32: 177 us, 5.9 TB/s, 91 % of the copy bandwidth; 4 CTAs an SM, 3 and 5 take 7 % and
+// (32,071 x 4,095 fp32: 171 us, 6.1 TB/s, 94 % of the copy bandwidth; 4 CTAs an SM, 3 and 5 take 7 % and
 // 15 % longer).
 // A vector is worked on as soon as it is there and its registers take the next batch's.
 // The entries at given columns are written once more, by the lane that holds the column.
@@ -949,7 +950,7 @@ __global__ void __launch_bounds__(32 * kWarps) score_short_backward_kernel(const
 
 template <typename T>
 cudaError_t launch_backward(const ScoreGradArgs& a, cudaStream_t st) {
-  // (300,000 x 63 fp32: 57 us, 264 by vectors; 120,000 x 255: 78 and 103)
+  // (300,000 x 63 fp32: 52 us, 264 by vectors; 120,000 x 255: 78 and 103)
   if (a.n_cols <= 256) {
     const auto ctas = [&](int g) { return (unsigned)((a.n_rows + 32 * kWarps / g - 1) / (32 * kWarps / g)); };
     if (a.n_cols <= 64) score_short_backward_kernel<T, 8, 8><<<ctas(8), 32 * kWarps, 0, st>>>(a);
@@ -971,7 +972,8 @@ cudaError_t launch_backward(const ScoreGradArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// By the row's length and the number of rows:
+// By the row's length and the number of rows (times between events around the call, L2 flushed: about 4 us
+// above the kernel's own):
 //  * up to 1,024 columns: the registers of a warp, or of 16 or 8 lanes where they hold the row
 //    and no more alternatives are asked for than lanes take part (300,000 x 63 fp32: 70 us, 161 with a
 //    warp a row; 200,000 x 127: 86 and 141; 60,000 x 511: 49 and 59);

@@ -1,8 +1,8 @@
 """The fitting step: the global norm of a list of gradients, clipping by it, and the Adam update.
 
-A fit of one family has two gradients, ``grad_theta`` [S, 3] and ``grad_col`` [S]; a fit of many families
-with rates of their own has two a family, and one norm over all of them.  There is no reference
-counterpart of these kernels (the reference's fits run torch optimisers).
+A solve has two gradients, ``grad_theta`` [S, 3] and ``grad_col`` [S].  A caller that fits several solves with
+rates of their own under one norm passes the gradients of all of them in one list.  There is no
+reference counterpart of these kernels (the reference's fits run torch optimisers).
 
     opt = fitting.Adam([theta], lr=0.05, max_norm=1.0)
     grad_theta, grad_col = runtime.run_backward(static, theta, col_weights, saved)
@@ -141,7 +141,8 @@ def _clip(source, destination, counts, n: int, kind: int, max_norm: float, like)
 
 def gradient_norm(grads, *, kind=2) -> torch.Tensor:
     """The norm of all entries of ``grads`` as one vector, a device scalar: the square root of the sum
-    of squares (``kind=2``) or the largest magnitude (``kind="max"``)."""
+    of squares (``kind=2``) or the largest magnitude (``kind="max"``).  It is returned in fp32 (infinite past
+    its range); clipping goes by the value in 64 bits."""
     kind = _kind(kind)
     grads = _sequence(grads)
     device = _device("grads", grads)
