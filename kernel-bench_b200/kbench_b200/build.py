@@ -51,8 +51,6 @@ def build_host(force: bool = False) -> Path:
     if HOST.exists() and not force and newest <= HOST.stat().st_mtime and made_for.exists() \
             and made_for.read_text() == target:
         return HOST
-    HOST.unlink(missing_ok=True)  # whatever becomes of this: it is not of this source for this target
-
     import torch
     base = Path(torch.__file__).resolve().parent
     include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
@@ -62,6 +60,7 @@ def build_host(force: bool = False) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
+        HOST.unlink(missing_ok=True)  # not of this source for this target
         raise RuntimeError(f"{cmd[0]} failed ({res.returncode})")
     os.replace(str(HOST) + ".tmp", HOST)
     made_for.parent.mkdir(exist_ok=True)
