@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -51,15 +52,18 @@ PyObject* guarded(const F& f) {
 
 // What a kernel wrote to through its address counts as changed in place: the version by which autograd and
 // whoever remembers something of a tensor know it (inference tensors have none).  Views of one block share a
-// counter, which moves on once: a step of an atomic is most of what this costs (2,048 views 10 us, 18 one by one).
-void mark_written(const std::vector<const at::Tensor*>& ts) {
-  std::vector<uint32_t> was(ts.size());
-  const auto counter = [&](size_t i) -> const c10::VariableVersion& { return ts[i]->unsafeGetTensorImpl()->version_counter(); };
-  for (size_t i = 0; i < ts.size(); ++i)
-    if (counter(i).enabled()) was[i] = counter(i).current_version();
-  for (size_t i = 0; i < ts.size(); ++i)
-    if (counter(i).enabled() && counter(i).current_version() == was[i]) ts[i]->unsafeGetTensorImpl()->bump_version();
-}
+// counter, which moves on once, where it is still what it was: a step of an atomic is most of what this costs.
+struct Written {
+  std::vector<std::pair<at::TensorImpl*, uint32_t>> versions;  // as they are before the call
+  void add(const at::Tensor& t) {
+    at::TensorImpl* impl = t.unsafeGetTensorImpl();
+    if (impl->version_counter().enabled()) versions.emplace_back(impl, impl->version_counter().current_version());
+  }
+  void mark() const {
+    for (const auto& [impl, was] : versions)
+      if (impl->version_counter().current_version() == was) impl->bump_version();
+  }
+};
 
 struct Span {
   uintptr_t begin, end;
@@ -95,9 +99,9 @@ bool spans_meet(std::vector<Span>& spans, const std::vector<size_t>& list_ends, 
 // What is asked of lists of tensors.  The first n_written are written, the others read.
 struct Lists {
   size_t n = 0;
-  std::vector<std::vector<const at::Tensor*>> ts;
   std::vector<std::vector<int64_t>> ptrs;  // per list, as the C entry points take them
   std::vector<std::vector<int32_t>> dtypes;
+  Written written;
   std::vector<int64_t> counts;             // of the first list
   std::vector<int> flags;                  // what is unusual in each list
   bool same = false;                       // tensor i has the same shape in all
@@ -106,7 +110,7 @@ struct Lists {
 
   // False with a Python error set where a list holds something else.
   bool look(PyObject* const* lists, size_t n_lists, int device, int n_written, bool in_place) {
-    ts.resize(n_lists);
+    std::vector<std::vector<const at::Tensor*>> ts(n_lists);
     same = n_lists > 0;
     for (size_t l = 0; l < n_lists; ++l) {
       if (!unpack(lists[l], ts[l])) return false;
@@ -116,6 +120,7 @@ struct Lists {
     ptrs.resize(n_lists);
     dtypes.resize(n_lists);
     flags.assign(n_lists, 0);
+    written.versions.reserve(n * (size_t)std::max(n_written, 0));
     counts.assign(n, 0);
     std::vector<std::vector<Span>> spans(n_lists);
     for (size_t l = 0; l < n_lists; ++l) {
@@ -135,6 +140,7 @@ struct Lists {
       if (!t.is_contiguous()) flags[l] |= kStrided;
       const int64_t count = t.numel();
       if (l == 0) counts[i] = count;
+      if ((int)l < n_written) written.add(t);
       dtypes[l][i] = code < 0 ? 0 : code;
       if (count == 0) return;
       const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
@@ -224,7 +230,9 @@ PyObject* written(PyObject*, PyObject* list) {
   return guarded([&]() -> PyObject* {
     std::vector<const at::Tensor*> ts;
     if (!unpack(list, ts)) return nullptr;
-    mark_written(ts);
+    Written w;
+    for (const at::Tensor* t : ts) w.add(*t);
+    w.mark();
     Py_RETURN_NONE;
   });
 }
@@ -365,7 +373,11 @@ PyObject* score_rows_backward(PyObject*, PyObject* args) {
         rows.data_ptr(), rows.stride(0), dtype_code(rows.scalar_type()), R, (int)S, natural, stats, entropy,
         given ? reinterpret_cast<const long long*>(given->data_ptr()) : nullptr, n_given, gm, gg, ge, out.data_ptr(),
         out.stride(0), (void*)stream);
-    if (status == 0 && out_o != Py_None) mark_written({&out});
+    if (status == 0 && out_o != Py_None) {
+      Written w;
+      w.add(out);
+      w.mark();
+    }
     return Py_BuildValue("(iN)", status, out_o == Py_None ? wrap(out) : Py_NewRef(out_o));
   });
 }
@@ -403,7 +415,7 @@ PyObject* clip(PyObject*, PyObject* args) {
     const int status = reinterpret_cast<decltype(&kb_clip_gradients)>(fn)(
         src, write ? dst : nullptr, reinterpret_cast<const long long*>(x.counts.data()), x.dtypes[g].data(), (int)x.n, kind,
         max_norm, b.norm.data_ptr<float>(), b.ws.data_ptr(), bytes, (void*)stream);
-    if (status == 0 && write) mark_written(x.ts[0]);
+    if (status == 0 && write) x.written.mark();
     return Py_BuildValue("(iN)", status, wrap(b.norm));
   });
 }
@@ -430,8 +442,7 @@ PyObject* adam(PyObject*, PyObject* args) {
     const int status = reinterpret_cast<decltype(&kb_adam_step)>(fn)(
         at(0), at(3), at(1), at(2), reinterpret_cast<const long long*>(x.counts.data()), x.dtypes[3].data(), (int)x.n, lr,
         b1, b2, eps, wd, c1, c2, kind, max_norm, b.norm.data_ptr<float>(), b.ws.data_ptr(), bytes, (void*)stream);
-    if (status == 0)
-      for (size_t l = 0; l < 3; ++l) mark_written(x.ts[l]);
+    if (status == 0) x.written.mark();
     return Py_BuildValue("(iN)", status, wrap(b.norm));
   });
 }
